@@ -21,9 +21,10 @@
 // row) and one byte permute per pair of rows transposes them.  No LDS and no cross-lane traffic but
 // the maximum of a column over its four lane groups.
 //
-// Accuracy: the running maximum, sum and output are f32.  q and the probabilities go to the matrix
-// cores as NS 16-bit parts (f32 activations: two f16 or three bf16 parts, 22 bits and more), q first
-// scaled by a power of two into f16's range; e4m3 codes are exact in f16.
+// Accuracy: the running maximum, sum and output are f32.  q and the weights go to the matrix cores as NS 16-bit
+// parts (f32 activations: two f16 or three bf16 parts), q first scaled by a power of two into f16's range (22
+// bits and more of a row's largest element), weights as PagedWeights says (19 bits and more of each); e4m3
+// codes are exact in f16.
 //
 // Measured with the join, 8 kv heads of 128 with 4 query heads each: 1 sequence of 131071 positions bf16 106 us (5.1
 // TB/s), 64 of up to 12000 e4m3 158 us (5.1 TB/s), 32 of up to 4096
@@ -79,6 +80,7 @@ struct PagedDecode {
     static constexpr bool TWO = HD <= 128;
     static constexpr int WAVES = paged_waves(HD, HD * ES, MULTI);
     static constexpr int WG = paged_wg(MULTI);  // waves of a worker
+    using Weights = PagedWeights<BF, NS>;
 
     struct Unit {
         uint32_t k[2][KS][KW];
@@ -307,7 +309,23 @@ struct PagedDecode {
             pv_odd<EE + 1>(st, u, sees, at, g);
         }
     }
-
+    static __device__ __forceinline__ void scale(State& st, int j, float by) {
+        st.l[j] *= by;
+#pragma unroll
+        for (int e = 0; e < E; e++) st.o[j][e] *= by;
+    }
+    // By how much group j's sums may rise, `want` at most.
+    static __device__ __forceinline__ float room(const State& st, int j, float want) {
+        float sum = max_x32(max_x16(st.l[j])), r = Weights::room_weights(sum);
+        if (__any(r < want)) {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) sum = fmaxf(sum, fabsf(st.o[j][e][i]));
+            r = Weights::room(max_x32(max_x16(sum)));
+        }
+        return fmaxf(0.f, fminf(r, want));
+    }
     static __device__ __forceinline__ void step(State& st, const pg_u4* q_s, Unit& u, const PagedAttnArgs& a,
                                                 const PagedRange& r, int cg, int t, int g, int c) {
         pg_f4 s[NC][2];
@@ -348,52 +366,6 @@ struct PagedDecode {
                 }
             }
         }
-        pg_u4 p[NC][NS];
-#pragma unroll
-        for (int j = 0; j < NC; j++) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = s[j][e / 4][e % 4];
-            if (a.softcap > 0.f) {
-                const float inv = st.qf[j] / a.softcap, up = a.softcap * kLog2e;
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = tanhf(x[e] * inv) * up;
-            }
-            const float f = a.softcap > 0.f ? 1.f : st.qf[j];
-            if (edge) {
-                int cc = c;
-                asm volatile("" : "+v"(cc));  // (worked out here, not kept over the loop)
-                const Column k = column(a, r, NC * cg + j, cc);
-                const int lo = k.lo - 32 * t - 4 * g, hi = k.hi - 32 * t - 4 * g;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int at = 16 * (e / 4) + e % 4;
-                    x[e] = (!MULTI || (at >= lo && at < hi)) && (u.ok >> e & 1) ? x[e] : -INFINITY;
-                }
-            }
-            float mx = x[0];
-#pragma unroll
-            for (int e = 1; e < 8; e++) mx = fmaxf(mx, x[e]);
-            mx = max_x32(max_x16(mx)) * f;
-            if (__any(mx > st.m[j] + kLazy)) {
-                mx = fmaxf(st.m[j], mx);
-                const float al = exp2_hw(st.m[j] - (mx == -INFINITY ? 0.f : mx));
-                st.l[j] *= al;
-#pragma unroll
-                for (int e = 0; e < E; e++) st.o[j][e] *= al;
-                st.m[j] = mx;
-            }
-            const float mm = st.m[j] == -INFINITY ? 0.f : st.m[j];
-#pragma unroll
-            for (int d = 0; d < 4; d++) {
-                const float p0 = exp2_hw(__builtin_fmaf(x[2 * d], f, -mm)), p1 = exp2_hw(__builtin_fmaf(x[2 * d + 1], f, -mm));
-                st.l[j] += p0 + p1;
-                uint32_t w[NS];
-                split2<BF, NS>(p0, p1, w);
-#pragma unroll
-                for (int n = 0; n < NS; n++) p[j][n][d] = w[n];
-            }
-        }
         if constexpr (MULTI) {
             if (edge && __any(odd_values(u))) {
 #pragma nounroll
@@ -410,7 +382,112 @@ struct PagedDecode {
                 drop_odd(u);
             }
         }
-        pv<0>(st, u, p);
+        float x[NC][8], least[NC];
+        bool bands = false;
+#pragma unroll
+        for (int j = 0; j < NC; j++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[j][e] = s[j][e / 4][e % 4];
+            if (a.softcap > 0.f) {
+                const float inv = st.qf[j] / a.softcap, most = a.softcap * kLog2e;
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[j][e] = tanhf(x[j][e] * inv) * most;
+            }
+            const float f = a.softcap > 0.f ? 1.f : st.qf[j];
+            if (edge) {
+                int cc = c;
+                asm volatile("" : "+v"(cc));  // (worked out here, not kept over the loop)
+                const Column k = column(a, r, NC * cg + j, cc);
+                const int lo = k.lo - 32 * t - 4 * g, hi = k.hi - 32 * t - 4 * g;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int at = 16 * (e / 4) + e % 4;
+                    x[j][e] = (!MULTI || (at >= lo && at < hi)) && (u.ok >> e & 1) ? x[j][e] : -INFINITY;
+                }
+            }
+            float mx = x[j][0], mn = x[j][0];
+#pragma unroll
+            for (int e = 1; e < 8; e++) mx = fmaxf(mx, x[j][e]);
+            if constexpr (!BF) {
+#pragma unroll
+                for (int e = 1; e < 8; e++) mn = fminf(mn, x[j][e]);
+                if (edge) {  // of the attended ones
+                    mn = INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) mn = fminf(mn, x[j][e] == -INFINITY ? INFINITY : x[j][e]);
+                }
+            }
+            mx = max_x32(max_x16(mx)) * f;
+            const bool under = Weights::under(mx, st.m[j]);
+            if (__any(under || Weights::above(mx, st.m[j]))) {
+                const float was = st.m[j];
+                st.m[j] = Weights::reference(mx, was);
+                if (__any(under)) {
+                    const float d = room(st, j, under ? was - ceilf(mx) : 0.f);
+                    if (under) st.m[j] = was - d;
+                }
+                scale(st, j, exp2_hw(was - (st.m[j] == -INFINITY ? 0.f : st.m[j])));
+            }
+            least[j] = INFINITY;
+            if constexpr (!BF) {
+                const float up = Weights::offset(st.m[j]), z = __builtin_fmaf(mn, f, up);
+                if (!Weights::far(st.m[j])) least[j] = z;
+                if (__any(least[j] < Weights::LEAST)) {
+                    float larger = 0.f, seen = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        larger += __builtin_fmaf(x[j][e], f, up) < Weights::LEAST ? 0.f : 1.f;
+                        seen += x[j][e] == -INFINITY ? 0.f : 1.f;
+                    }
+                    bands |= __any(least[j] < Weights::LEAST && Weights::few(sum_x32(sum_x16(larger)), sum_x32(sum_x16(seen))));
+                }
+            }
+        }
+        // The weights from 2^LEAST on; then, with the sums raised, those below, a band at a time (rare: PagedWeights).
+        float most[NC], raise = 0.f;  // by how much the sums of this lane's columns rise in the end; by now at most
+#pragma unroll
+        for (int j = 0; j < NC; j++) most[j] = bands ? Weights::wanted(max_x32(max_x16(-least[j]))) : 0.f;
+        for (;;) {
+            pg_u4 p[NC][NS];
+#pragma unroll
+            for (int j = 0; j < NC; j++) {
+                const float f = a.softcap > 0.f ? 1.f : st.qf[j], up = Weights::offset(st.m[j]) + raise;
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = x[j][e];
+                if (bands) {
+                    const float before = Weights::before(up, raise, most[j]);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) y[e] = Weights::other(x[j][e], f, up, before) ? -INFINITY : x[j][e];
+                }
+#pragma unroll
+                for (int d = 0; d < 4; d++) {
+                    const float p0 = exp2_hw(__builtin_fmaf(y[2 * d], f, up)), p1 = exp2_hw(__builtin_fmaf(y[2 * d + 1], f, up));
+                    st.l[j] += p0 + p1;
+                    uint32_t w[NS];
+                    split2<BF, NS>(p0, p1, w);
+#pragma unroll
+                    for (int n = 0; n < NS; n++) p[j][n][d] = w[n];
+                }
+            }
+            pv<0>(st, u, p);
+            if (!bands) break;
+            bool more = false;
+#pragma unroll
+            for (int j = 0; j < NC; j++) {
+                if (raise == 0.f) most[j] = Weights::whole(room(st, j, most[j]));
+                more |= raise < most[j];
+            }
+            if (!__any(more)) break;
+            again(u);
+#pragma unroll
+            for (int j = 0; j < NC; j++) scale(st, j, raise < most[j] ? exp2_hw(Weights::BAND) : 1.f);
+            raise += Weights::BAND;
+        }
+        if (bands) {
+#pragma unroll
+            for (int j = 0; j < NC; j++) scale(st, j, exp2_hw(-most[j]));
+        }
     }
 };
 
@@ -540,13 +617,13 @@ __global__ __launch_bounds__(64 * paged_wg(MULTI), (PagedDecode<HD, KT, NS, MULT
         if constexpr (WG == 1) {
             const float l = sum_x32(sum_x16(st.l[0]));
             if (16 * cg + c < r.rows) {
-                const float f = done ? (l == 0.f ? 0.f : vs / l) : 1.f;
+                const float f = done ? (l == 0.f ? 0.f : 1.f / l) : 1.f, fv = done ? vs : 1.f;
                 const long long entry = static_cast<long long>(slot) * a.cols + c;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     float x[E];
 #pragma unroll
-                    for (int e = 0; e < E; e++) x[e] = st.o[0][e][i] * f;
+                    for (int e = 0; e < E; e++) x[e] = st.o[0][e][i] * f * fv;
                     constexpr int V = E % 8 == 0 ? 8 : E % 4 == 0 ? 4 : 2;
                     const int d = (4 * g + i) * E;
                     if (done) {
@@ -595,9 +672,9 @@ __global__ __launch_bounds__(64 * paged_wg(MULTI), (PagedDecode<HD, KT, NS, MULT
                 }
                 if (done) {
                     const int R = 16 * NC * cg + col, tok = paged_div(R, a.rep_mul, a.rep_shift);
-                    const float f = l == 0.f ? 0.f : vs / l;
+                    o *= l == 0.f ? 0.f : 1.f / l;
                     act_store4<D::AF>(a.out, (r.row0 + tok) * a.out_ld + static_cast<long long>(h * a.reps + R - tok * a.reps) * HD + d,
-                                      a.act_type, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+                                      a.act_type, o[0] * vs, o[1] * vs, o[2] * vs, o[3] * vs);
                 } else {
                     const long long entry = static_cast<long long>(slot) * a.cols + col;
                     *reinterpret_cast<pg_f4*>(a.part + entry * HD + d) = o;
@@ -652,7 +729,7 @@ __global__ __launch_bounds__(TH) void paged_decode_join_kernel(PagedAttnArgs a) 
         float m = -INFINITY, l = 0.f;
         for (int i = lane; i < n; i += 64) m = fmaxf(m, ml(i, c).x);
         m = wave_max(m);
-        const float mm = m == -INFINITY ? 0.f : m;
+        const float mm = (m == -INFINITY ? 0.f : m) + kJoinDown;
         for (int i = lane; i < n; i += 64) l += ml(i, c).y * exp2_hw(ml(i, c).x - mm);
         l = wave_sum(l);
         if (lane == 0) ml_s[c] = make_float2(mm, l);
@@ -673,8 +750,8 @@ __global__ __launch_bounds__(TH) void paged_decode_join_kernel(PagedAttnArgs a) 
     for (int j = 1; j < PG; j++) o += o_s[k + j * a.join_cols][d];
     const float l = ml_s[col].y;
     const float vs = a.kv_type == LARQL_ELEM_E4M3 && a.c.v_scale ? a.c.v_scale[h] : 1.f;
-    const float f = l == 0.f ? 0.f : vs / l;
-    act_store4<AF>(a.out, out, a.act_type, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+    o *= l == 0.f ? 0.f : 1.f / l;
+    act_store4<AF>(a.out, out, a.act_type, o[0] * vs, o[1] * vs, o[2] * vs, o[3] * vs);
 }
 
 template <int HD, bool MULTI>

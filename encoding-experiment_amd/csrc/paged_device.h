@@ -253,10 +253,65 @@ __device__ __forceinline__ float sum_x16(float v) {
 // 2^x on the hardware's unit (1 ulp; results below 2^-126 become 0).
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The reference of a row's exponentials follows its maximum only where that rose by more than this
-// (log2): the sums then stay below 2^8 times the terms, which f32 (and f16 probabilities) hold as well, and
-// most tiles rescale nothing.
-constexpr float kLazy = 8.f;
+// A row's weights 2^(s - m) (s: its scores in log2, m: its reference) on their way to the matrix cores as NS 16-bit
+// parts.  m is a whole number, so that rescaling the sums rounds nothing, and follows the row's largest score only where
+// that rose by more than LAZY, so that most tiles rescale nothing.
+//
+// bf16 parts have f32's range.  f16 ends at 2^-24, so there weights are taken as 2^(z = s - m + UP) (the sums l too: it
+// cancels in the end), and the parts hold those from 2^LEAST on: two of them to half a step of 2^-24, 2^-19 of the
+// weight; one to its own rounding (the least normal number is 2^-14).  Smaller ones are held to 2^-25, 2^-39 of the
+// row's largest.  That is too little where the larger ones meet values near zero, as an attention sink's are:
+// - a tile whose largest weight is below 2^LOW lets m fall to its largest score (the sums rise with it, exactly, up to
+//   2^MOST), so the tiles behind a position that dominates a row are like any others;
+// - in a tile where FEW weights or a quarter of them (one at least) are not too small, the others are summed apart: decode in
+//   bands of BAND, each with the sums raised as far; prompts, where a second set of products next to the first cost
+//   every tile 10-40%, in f32 without the matrix cores.
+// With more of them the others stay as they are: taking those apart too cost rows whose scores are spread widely (3 nats
+// deviation) 2 to 5 times the time, for a case in which all of the larger values would have to be near zero.
+// 512 tokens f32 over f16 33.3 us, 41 with a sink 18 nats above the rest, 41 with scores of 3 nats deviation; 32 sequences'
+// decode 53 us in all three.  Without any of it 30 us and 52, and errors of 1e-3 behind a sink of 12 nats, 0.4 at 18.
+template <bool BF, int NS>
+struct PagedWeights {
+    static constexpr float UP = BF ? 0.f : 14.f, LAZY = BF ? 8.f : 1.98f;  // (2^15.98 is f16's largest)
+    static constexpr float LEAST = NS == 1 ? -14.f : -6.f, BAND = UP - LEAST, LOW = 5.f, FEW = 4.f;
+    static constexpr float MOST = 122.f;  // (four lanes' or waves' sums of that stay finite)
+
+    // Scores past 2^16 round by more than there is room above the largest weight: theirs start lower, and rise by nothing.
+    static __device__ __forceinline__ bool far(float m) { return fabsf(m) > 65536.f; }
+    // Whether a tile's largest score mx calls for a higher reference, and that one; or for a lower one.
+    static __device__ __forceinline__ bool above(float mx, float m) { return mx > m + (far(m) ? -UP : LAZY); }
+    static __device__ __forceinline__ float reference(float mx, float m) {
+        return fmaxf(m, ceilf(mx) + (far(mx) ? UP : 0.f));
+    }
+    static __device__ __forceinline__ bool under(float mx, float m) {
+        return !BF && mx - m + UP < LOW && mx != -INFINITY && !far(m) && !far(mx);
+    }
+    // By how much (log2) sums of up to `sum` may rise; with values below 2^16 and four lanes' sums of the weights, l.
+    static __device__ __forceinline__ float room(float sum) { return MOST - __builtin_amdgcn_frexp_expf(sum); }
+    static __device__ __forceinline__ float room_weights(float l) { return room(l) - 18.f; }
+    // What they have to rise by for weights of z = -below (none past -126) to be in reach, whatever its rounding; whole
+    // bands of that.
+    static __device__ __forceinline__ float wanted(float below) {
+        return BAND * ceilf((fminf(below, 126.f) + LEAST + 0.01f) / BAND);
+    }
+    static __device__ __forceinline__ float whole(float rise) { return BAND * floorf(rise / BAND); }
+    // What z is for a score of 0.
+    static __device__ __forceinline__ float offset(float m) { return UP - (m == -INFINITY ? 0.f : m); }
+    // A tile whose sums rise by `most`, whole bands, in passes as `raise` goes up by BAND: the offset `up` of a pass is that
+    // without a rise + raise.  Of the pass before (infinite: there is none; all is done):
+    static __device__ __forceinline__ float before(float up, float raise, float most) {
+        return raise == 0.f ? -INFINITY : raise <= most ? up - BAND : INFINITY;
+    }
+    // Whether `larger` of a tile's `seen` weights, those that are not too small, are few.
+    static __device__ __forceinline__ bool few(float larger, float seen) { return larger <= fmaxf(1.f, fminf(FEW, 0.25f * seen)); }
+    // Whether a product x (score = x f) is none of the pass at offset up: too small for it, or done at the one before.
+    static __device__ __forceinline__ bool other(float x, float f, float up, float before) {
+        return __builtin_fmaf(x, f, up) < LEAST || __builtin_fmaf(x, f, before) >= LEAST;
+    }
+};
+
+// Joined parts are taken down by 2^kJoinDown: as many sums as high as they go stay finite.
+constexpr float kJoinDown = 12.f;
 
 // Scores are products times `f` >= 0: the query takes the scale's sign, and f stays large enough that a
 // masked product of -inf is a score of -inf (products are below 2^50: at 1e-37 they count as 0).

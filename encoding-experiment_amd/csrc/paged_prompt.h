@@ -39,12 +39,13 @@ struct PagedPrompt {
     static constexpr int ES = KT == LARQL_ELEM_E4M3 ? 1 : 2;
     static constexpr int KV = 64;  // positions per tile: one to a lane
     // Scores held at once, in 32s: a whole tile's, or half of them where several parts of the rows leave no room.
-    static constexpr int JN = (HD > 96 && NS == 2) || (HD > 128 && NS == 3) ? 1 : KV / 32;
+    static constexpr int JN = (HD > (KT == LARQL_ELEM_E4M3 ? 64 : 96) && NS == 2) || (HD > 128 && NS == 3) ? 1 : KV / 32;
     static constexpr int NC = HD / 8;               // 16-byte pieces of an LDS row
     static constexpr int CH = KV * NC / 256;          // pieces per thread of one tile
     static constexpr bool DIRECT = ES == 2;           // pieces go from memory to LDS as they are
     static constexpr int KS = HD / 16, DT = HD / 32;
     static constexpr int W = 2 * ES;              // words of a piece in the cache
+    using Weights = PagedWeights<BF, NS>;
     // Three parts of a wide row are more registers than the row itself: it stays f32, split per use.
     static constexpr bool QF = NS == 3 && HD > 192;
 
@@ -365,7 +366,8 @@ __global__ __launch_bounds__(256, HD <= 128 && NS <= 2 ? 2 : 1) void paged_promp
             const int j0 = 32 * JN * jb, p0 = it * KV + j0;  // rows of the tile, positions
             const bool go = busy && p0 <= w_hi && p0 + 32 * JN - 1 > w_lo - win;
             pg_f16 s[JN];  // 32 positions each
-            float f, mm;
+            float f, up;         // weights: 2^(s f + up)
+            bool small = false;  // some are too small for the parts
             if (go) {
                 const int row = here(n);
                 pg_u4 kf[JN][KS];
@@ -412,13 +414,15 @@ __global__ __launch_bounds__(256, HD <= 128 && NS <= 2 ? 2 : 1) void paged_promp
                     all &= ok[j];
                 }
                 if (a.softcap > 0.f) {
-                    const float inv = qf / a.softcap, up = a.softcap * kLog2e;
+                    const float inv = qf / a.softcap, most = a.softcap * kLog2e;
 #pragma unroll
                     for (int j = 0; j < JN; j++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) s[j][e] = tanhf(s[j][e] * inv) * up;
+                        for (int e = 0; e < 16; e++) s[j][e] = tanhf(s[j][e] * inv) * most;
                 }
+                float mn = s[0][0];
                 if (p0 + 32 * JN - 1 > w_lo || p0 <= w_hi - win || ~all) {
+                    mn = INFINITY;
 #pragma unroll
                     for (int j = 0; j < JN; j++) {
                         const int hi = tq - p0 - 32 * j - 4 * hh, lo = hi - win;
@@ -426,9 +430,16 @@ __global__ __launch_bounds__(256, HD <= 128 && NS <= 2 ? 2 : 1) void paged_promp
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
                             const int at = 8 * (e / 4) + e % 4;  // position p0 + 32 j + 4 hh + at
-                            s[j][e] = at <= hi && at > lo && (okh >> at & 1) ? s[j][e] : -INFINITY;
+                            const bool in = at <= hi && at > lo && (okh >> at & 1);
+                            if constexpr (!BF) mn = fminf(mn, in ? s[j][e] : INFINITY);
+                            s[j][e] = in ? s[j][e] : -INFINITY;
                         }
                     }
+                } else if constexpr (!BF) {
+#pragma unroll
+                    for (int j = 0; j < JN; j++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) mn = fminf(mn, s[j][e]);
                 }
                 f = a.softcap > 0.f ? 1.f : qf;
                 float mx = s[0][0];
@@ -437,15 +448,17 @@ __global__ __launch_bounds__(256, HD <= 128 && NS <= 2 ? 2 : 1) void paged_promp
 #pragma unroll
                     for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[j][e]);
                 mx = max_x32(mx) * f;
-                if (__any(mx > m + kLazy)) {
-                    mx = fmaxf(m, mx);
-                    const float al = exp2_hw(m - (mx == -INFINITY ? 0.f : mx));
+                const bool under = P::Weights::under(mx, m);
+                if (__any(under || P::Weights::above(mx, m))) {
+                    const float was = m, room = P::Weights::room_weights(max_x32(l));
+                    m = under ? was - fmaxf(0.f, fminf(was - ceilf(mx), room)) : P::Weights::reference(mx, was);
+                    const float al = exp2_hw(was - (m == -INFINITY ? 0.f : m));
                     l *= al;
 #pragma unroll
                     for (int d = 0; d < DT; d++) o[d] *= al;
-                    m = mx;
                 }
-                mm = m == -INFINITY ? 0.f : m;
+                up = P::Weights::offset(m);
+                if constexpr (!BF) small = __any(__builtin_fmaf(mn, f, up) < P::Weights::LEAST && !P::Weights::far(m));
             }
             if (__builtin_amdgcn_readfirstlane(bad) == it) {  // (the same for the workgroup)
                 if (go)
@@ -474,12 +487,67 @@ __global__ __launch_bounds__(256, HD <= 128 && NS <= 2 ? 2 : 1) void paged_promp
                 }
                 __syncthreads();
             }
+            if (!BF && small) {
+                // Weights too small for the parts, in rows where they are most of a tile's: summed here in f32, left out below.
+                float larger = 0.f, seen = 0.f;
+#pragma unroll
+                for (int j = 0; j < JN; j++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        larger += __builtin_fmaf(s[j][e], f, up) < P::Weights::LEAST ? 0.f : 1.f;
+                        seen += s[j][e] == -INFINITY ? 0.f : 1.f;
+                    }
+                const bool few = P::Weights::few(sum_x32(larger), sum_x32(seen));
+                if (__any(few)) {
+#pragma unroll
+                    for (int j = 0; j < JN; j++)
+#pragma nounroll
+                        for (int e = 0; e < 16; e++) {
+                            const float z = __builtin_fmaf(s[j][0], f, up);
+                            const bool mine = few && z < P::Weights::LEAST;
+                            const float p = exp2_hw(mine ? z : -INFINITY), y = mine ? -INFINITY : s[j][0];
+                            l += p;
+#pragma unroll
+                            for (int i = 0; i < 15; i++) s[j][i] = s[j][i + 1];  // (registers have no index)
+                            s[j][15] = y;
+                            if (!__any(p > 0.f)) continue;
+                            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(p), __float_as_uint(p), false, false);
+                            float pk = __uint_as_float(both[0]), pn = __uint_as_float(both[1]);  // of the lanes' lower, upper half
+#pragma nounroll
+                            for (int k = 0; k < 2; k++) {
+                                const int at = j0 + 32 * j + 8 * (e / 4) + e % 4 + 4 * k;
+                                auto value = [&](int i) __attribute__((always_inline)) {  // dims 8 i + 4 hh ..
+                                    return reinterpret_cast<const uint2*>(&v_s[buf][at * NC + P::swz_v(at, i)])[hh];
+                                };
+                                uint2 w[2][4];
+#pragma unroll
+                                for (int i = 0; i < 4; i++) w[0][i] = value(i);
+#pragma unroll
+                                for (int d = 0; d < DT; d++) {
+#pragma unroll
+                                    for (int i = 0; i < 4; i++)
+                                        if (d + 1 < DT) w[(d + 1) & 1][i] = value(4 * (d + 1) + i);
+#pragma unroll
+                                    for (int i = 0; i < 4; i++) {
+                                        const uint2 v = w[d & 1][i];
+                                        o[d][4 * i] += pk * unpack_lo<BF>(v.x);
+                                        o[d][4 * i + 1] += pk * unpack_hi<BF>(v.x);
+                                        o[d][4 * i + 2] += pk * unpack_lo<BF>(v.y);
+                                        o[d][4 * i + 3] += pk * unpack_hi<BF>(v.y);
+                                    }
+                                    __builtin_amdgcn_sched_barrier(0);  // (two blocks' values at a time)
+                                }
+                                pk = pn;
+                            }
+                        }
+                }
+            }
             if (go) {
                 uint32_t pw[JN][NS][8];
                 auto weights = [&](int j) {
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        const float x0 = exp2_hw(__builtin_fmaf(s[j][e], f, -mm)), x1 = exp2_hw(__builtin_fmaf(s[j][e + 1], f, -mm));
+                        const float x0 = exp2_hw(__builtin_fmaf(s[j][e], f, up)), x1 = exp2_hw(__builtin_fmaf(s[j][e + 1], f, up));
                         l += x0 + x1;
                         uint32_t w[NS];
                         split2<BF, NS>(x0, x1, w);
@@ -530,13 +598,13 @@ __global__ __launch_bounds__(256, HD <= 128 && NS <= 2 ? 2 : 1) void paged_promp
     const long long row = t.row0 + tok;
     const float vs = KT == LARQL_ELEM_E4M3 && a.c.v_scale ? a.c.v_scale[h] : 1.f;
     if (a.splits == 1) {
-        const float f = l == 0.f ? 0.f : vs / l;
+        const float f = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
                 act_store4<AF>(a.out, row * a.out_ld + static_cast<long long>(head) * HD + 32 * d + 2 * e + 4 * hh, a.act_type,
-                           o[d][e] * f, o[d][e + 1] * f, o[d][e + 2] * f, o[d][e + 3] * f);
+                           o[d][e] * f * vs, o[d][e + 1] * f * vs, o[d][e + 2] * f * vs, o[d][e + 3] * f * vs);
     } else {
         const long long at = (row * a.num_q + head) * a.splits + blockIdx.y;
         if (hh == 0) *reinterpret_cast<float2*>(a.tile_ml + 2 * at) = make_float2(m, l);
@@ -571,7 +639,7 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedAttnArgs a)
     if (row < row0 || row >= row0 + n || n * a.reps <= a.few) return;
     float m = -INFINITY, l = 0.f;
     for (int s = 0; s < a.splits; s++) m = fmaxf(m, a.tile_ml[2 * (i * a.splits + s)]);
-    const float mm = m == -INFINITY ? 0.f : m;
+    const float mm = (m == -INFINITY ? 0.f : m) + kJoinDown;
     pg_f4 o = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < a.splits; s++) {
         const float2 p = *reinterpret_cast<const float2*>(a.tile_ml + 2 * (i * a.splits + s));
@@ -581,9 +649,9 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedAttnArgs a)
         o += *reinterpret_cast<const pg_f4*>(a.tile_part + (i * a.splits + s) * HD + 4 * d) * f;
     }
     const float vs = a.kv_type == LARQL_ELEM_E4M3 && a.c.v_scale ? a.c.v_scale[head / a.reps] : 1.f;
-    const float f = l == 0.f ? 0.f : vs / l;
-    act_store4<AF>(a.out, row * a.out_ld + static_cast<long long>(head) * HD + 4 * d, a.act_type, o[0] * f, o[1] * f, o[2] * f,
-               o[3] * f);
+    o *= l == 0.f ? 0.f : 1.f / l;
+    act_store4<AF>(a.out, row * a.out_ld + static_cast<long long>(head) * HD + 4 * d, a.act_type, o[0] * vs, o[1] * vs, o[2] * vs,
+               o[3] * vs);
 }
 
 template <int HD>
