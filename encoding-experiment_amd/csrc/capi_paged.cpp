@@ -172,7 +172,7 @@ extern "C" int larql_hip_paged_attention_work_bytes(larql_hip_ctx* c, const larq
     return guarded(c, [&] {
         need(bytes, "null bytes");
         larql::PagedAttnArgs a = make_attn(cache, batch, num_q_heads, false);
-        *bytes = batch->num_tokens ? larql::paged_attn_plan(a, nullptr, c->num_cus) : 0;
+        *bytes = batch->num_tokens ? larql::paged_attn_most(a, c->num_cus) : 0;
     });
 }
 

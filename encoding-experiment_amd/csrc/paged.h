@@ -103,6 +103,9 @@ constexpr int paged_waves(int hd, int row, bool multi) {
 void launch_paged_append(const PagedAppendArgs& a, hipStream_t s);
 // Work buffer bytes of one attention call, and the pointers of `a` into it (work null: sizes only).
 size_t paged_attn_plan(PagedAttnArgs& a, void* work, int num_cus);
+// What is enough for one call of every batch of no more sequences, tokens and positions over the same cache (with q_start:
+// also without).  A prompt of fewer tokens takes more parts, so one call's own is not.
+size_t paged_attn_most(PagedAttnArgs a, int num_cus);
 void launch_paged_attention(const PagedAttnArgs& a, hipStream_t s);
 
 // One launcher per head_dim (each compiled in a file of its own), by cache type and activation type.

@@ -717,7 +717,8 @@ class HipBackend:
             hd ** -0.5 if scale is None else scale, window, softcap, wp, n, _stream_ptr(stream)))
 
     def paged_attention_work_bytes(self, cache: PagedKV, batch: PagedBatch, num_q_heads: int) -> int:
-        """Bytes of work buffer that paged_attention_dev needs for these shapes."""
+        """Bytes of work buffer that paged_attention_dev needs for these shapes, and for every batch of no
+        more sequences, tokens and table pages (asked for with q_start, also without)."""
         n = _SZ()
         self._check(self._lib.larql_hip_paged_attention_work_bytes(self._ctx, cache._ref, batch._ref, num_q_heads,
                                                                    ctypes.byref(n)))

@@ -550,7 +550,9 @@ int larql_hip_paged_attention_dev(larql_hip_ctx* ctx, const larql_paged_kv* cach
                                   int type, const void* q, size_t q_stride, size_t num_q_heads, void* out,
                                   size_t out_stride, float scale, size_t window, float softcap, void* work,
                                   size_t work_bytes, void* stream);
-/* Bytes of work buffer for a cache and batch of these shapes (contents are not read). */
+/* Bytes of work buffer for a cache and batch of these shapes (contents are not read).  Enough for every batch of
+ * no more sequences, tokens and table pages over a cache of the same type, heads, head_dim and page_size;
+ * asked for with q_start, also for those without. */
 int larql_hip_paged_attention_work_bytes(larql_hip_ctx* ctx, const larql_paged_kv* cache,
                                          const larql_paged_batch* batch, size_t num_q_heads, size_t* bytes);
 
