@@ -676,7 +676,8 @@ class HipBackend:
                          rotary_dim: int = 0, stream=None):
         """Stores the batch's new keys and values [tokens][kv_heads][head_dim] into their pages, keys
         rotated by their positions, and writes the rotated queries to q_out (None: into q).  rope_base 0: no
-        rotation; rotary_dim 0: the whole head."""
+        rotation; rotary_dim 0: the whole head.  stream: the torch stream on which the tensors are made and read
+        (None: the context's own, in no order with torch's)."""
         self._paged(cache, batch)
         T, hd, nkv, kind = batch.tokens, cache.head_dim, cache.num_kv_heads, k.dtype
         heads = qs = os_ = 0
@@ -699,7 +700,8 @@ class HipBackend:
                             softcap: float = 0.0, stream=None):
         """Attention of the batch's token rows q [tokens][heads][head_dim] over their sequences' pages
         (causal, the last `window` positions if set) into out.  scale None: head_dim ** -0.5.  work: a
-        16-byte aligned device buffer of paged_attention_work_bytes, this call's alone until it has run."""
+        16-byte aligned device buffer of paged_attention_work_bytes, this call's alone until it has run.  stream: the
+        torch stream on which the tensors are made and read (None: the context's own, in no order with torch's)."""
         self._paged(cache, batch)
         T, hd = batch.tokens, cache.head_dim
         heads = q.shape[1] if q.dim() == 3 else q.shape[-1] // hd
