@@ -180,13 +180,23 @@ def prepare(case, seed):
         s["be"] = be
         s["kv"] = larql_hip.PagedKV(s["k_pages"], s["v_pages"], s.get("k_scale"), s.get("v_scale"))
         s["batch"] = larql_hip.PagedBatch(s["table"], s["kv_len"], s["q_start"], tokens=T)
+        s["stream"] = _stream()
         if c["kind"] != "append":
             n = be.paged_attention_work_bytes(s["kv"], s["batch"], nq)
             s["work"] = torch.empty(max(16, n), device="cuda", dtype=torch.uint8)
+        s["stream"].wait_stream(torch.cuda.current_stream())  # what was made above
     return s
 
 
 _be = None
+_streams = []
+
+
+def _stream():
+    """The one stream of every pass, as in a serving loop."""
+    if not _streams:
+        _streams.append(torch.cuda.Stream())
+    return _streams[0]
 
 
 def _backend():
@@ -206,12 +216,12 @@ def run(state):
             nq, nkv, hd = s["nq"], s["nkv"], s["hd"]
             q, k, v = s["qkv"].split([nq * hd, nkv * hd, nkv * hd], dim=1)
             s["be"].paged_append_dev(s["kv"], s["batch"], k, v, q=q, q_out=s["out"], rope_base=s["base"],
-                                     rotary_dim=c["rotary"])
+                                     rotary_dim=c["rotary"], stream=s["stream"])
             return s["k_pages"], s["v_pages"], s["out"]
         return _plain_append(s)
     if own:
         s["be"].paged_attention_dev(s["kv"], s["batch"], s["q"], s["out"], scale=s["hd"] ** -0.5, window=c["window"],
-                                    softcap=c["softcap"], work=s["work"])
+                                    softcap=c["softcap"], work=s["work"], stream=s["stream"])
         return s["out"]
     return _plain_attention(s)
 
