@@ -43,6 +43,25 @@ size_t rows_bytes(size_t rows, size_t stride, size_t width, int type) {
     return rows ? ((rows - 1) * stride + width) * elem_bytes(type) : 0;
 }
 
+// Whether [a, a + na) meets the pages at p: blocks of a page's positions and heads, `page` bytes apart (what lies between
+// them, as in one allocation for several layers, is not theirs).
+bool meets_pages(const void* p, size_t page, size_t pos, size_t head, const larql_paged_kv* kv, const void* a, size_t na) {
+    using wide = unsigned __int128;
+    const size_t es = elem_bytes(kv->type);
+    const wide x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(a), stride = page * es;
+    const wide block = ((kv->page_size - 1) * static_cast<wide>(pos) + (kv->num_kv_heads - 1) * static_cast<wide>(head) + kv->head_dim) * es;
+    const wide all = (kv->num_pages - 1) * stride + block;
+    if (na == 0 || y >= x + all || x >= y + na) return false;
+    if (y <= x || kv->num_pages == 1 || block >= stride) return true;
+    const wide at = (y - x) % stride;
+    return at < block || ((y - x) / stride + 1 < kv->num_pages && at + na > stride);
+}
+void check_pages(const larql_paged_kv* kv, const void* a, size_t na, const char* what) {
+    need(!meets_pages(kv->k, kv->k_page_stride, kv->k_pos_stride, kv->k_head_stride, kv, a, na) &&
+             !meets_pages(kv->v, kv->v_page_stride, kv->v_pos_stride, kv->v_head_stride, kv, a, na),
+         what);
+}
+
 // `pages`: the page memory itself is needed (else only the shapes).
 larql::PagedView make_view(const larql_paged_kv* kv, const larql_paged_batch* bt, bool pages) {
     need(kv && bt, "null cache or batch");
@@ -134,10 +153,14 @@ extern "C" int larql_hip_paged_append_dev(larql_hip_ctx* c, const larql_paged_kv
         if (T == 0) return;
         check_rows(k, k_stride, kvd, type, "k");
         check_rows(v, v_stride, kvd, type, "v");
+        check_pages(cache, k, rows_bytes(T, k_stride, kvd, type), "k overlaps the pages");
+        check_pages(cache, v, rows_bytes(T, v_stride, kvd, type), "v overlaps the pages");
         if (q) {
             check_rows(q, q_stride, qd, type, "q");
             check_rows(q_out, q_out_stride, qd, type, "q_out");
             const size_t no = rows_bytes(T, q_out_stride, qd, type);
+            check_pages(cache, q, rows_bytes(T, q_stride, qd, type), "q overlaps the pages");
+            check_pages(cache, q_out, no, "q_out overlaps the pages");
             // (rows of a packed projection interleave: equal strides whose rows do not meet are fine)
             auto rows_meet = [&](const void* p, size_t stride, size_t width) {
                 if (!overlap(q_out, no, p, rows_bytes(T, stride, width, type))) return false;
@@ -189,7 +212,9 @@ extern "C" int larql_hip_paged_attention_dev(larql_hip_ctx* c, const larql_paged
         if (T == 0) return;
         check_rows(q, q_stride, qd, type, "q");
         check_rows(out, out_stride, qd, type, "out");
-        need(!overlap(q, rows_bytes(T, q_stride, qd, type), out, rows_bytes(T, out_stride, qd, type)), "out overlaps q");
+        const size_t nq = rows_bytes(T, q_stride, qd, type), no = rows_bytes(T, out_stride, qd, type);
+        need(!overlap(q, nq, out, no), "out overlaps q");
+        check_pages(cache, out, no, "out overlaps the pages");
         a.act_type = type;
         a.q = q;
         a.out = out;
@@ -201,6 +226,8 @@ extern "C" int larql_hip_paged_attention_dev(larql_hip_ctx* c, const larql_paged
         const size_t bytes = larql::paged_attn_plan(a, work, c->num_cus);
         need(bytes == 0 || (work && aligned16(work)), "work is null or not 16-byte aligned");
         need(work_bytes >= bytes, "work buffer too small (larql_hip_paged_attention_work_bytes)");
+        need(!overlap(work, bytes, q, nq) && !overlap(work, bytes, out, no), "work overlaps q or out");
+        check_pages(cache, work, bytes, "work overlaps the pages");
         larql::launch_paged_attention(a, pick_stream(c, stream));
     });
 }

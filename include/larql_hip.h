@@ -525,7 +525,8 @@ typedef struct {
  * head turn as split halves by position * rope_base^(-2 j / rotary_dim) (LI/src/attention/rope.rs:
  * 22-55; angles in f64); rope_base 0: no rotation.  Stored values are rounded to nearest even once;
  * E4M3 ones are x * (1 / scale), saturated at +-448 (NaN stays NaN).  q NULL (num_q_heads 0): keys
- * and values only.  q_out may be q itself (same stride).  A position below 0 or without a page
+ * and values only.  q_out may be q itself (same stride); otherwise it overlaps none of the others, and nothing
+ * overlaps the pages.  A position below 0 or without a page
  * stores nothing, its q row is still rotated.  Two tokens of one call must not share a slot. */
 int larql_hip_paged_append_dev(larql_hip_ctx* ctx, const larql_paged_kv* cache, const larql_paged_batch* batch,
                                int type, const void* q, size_t q_stride, size_t num_q_heads, const void* k,
@@ -538,7 +539,7 @@ int larql_hip_paged_append_dev(larql_hip_ctx* ctx, const larql_paged_kv* cache, 
  * head i / (num_q_heads / num_kv_heads).  A row that attends nothing (kv_len 0, no pages) gives
  * zeros.  Whatever lies in positions a row does not attend (NaN and infinities too) has no effect; a
  * value that is not finite in one it does attend makes that dim of the row not finite.
- * q, out as for the append, not overlapping.  Results do not depend on the run: no atomics.
+ * q, out as for the append; q, out, work and the pages do not overlap.  Results do not depend on the run: no atomics.
  * Softmax statistics and sums are f32.  f32 activations are taken to f32 accuracy over every cache
  * type (f16 and E4M3 pages: each weight to 2^-19 down to 2^-20 of the largest one, and below that
  * where at most four positions of 32 are larger; else to 2^-39 of the row's largest); with 16-bit ones
