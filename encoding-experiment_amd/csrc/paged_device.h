@@ -313,9 +313,9 @@ struct PagedWeights {
 // Joined parts are taken down by 2^kJoinDown: as many sums as high as they go stay finite.
 constexpr float kJoinDown = 12.f;
 
-// Scores are products times `f` >= 0: the query takes the scale's sign, and f stays large enough that a
-// masked product of -inf is a score of -inf (products are below 2^50: at 1e-37 they count as 0).
-__device__ __forceinline__ float score_factor(float f) { return fmaxf(fabsf(f), 1e-37f); }
+// Scores are products times `f` >= 0: the query takes the scale's sign, and f stays above 0, so that a masked product
+// of -inf is a score of -inf (of products up to 10^38, over bf16 pages, the least f makes 0).
+__device__ __forceinline__ float score_factor(float f) { return fmaxf(fabsf(f), 1.4e-45f); }
 
 // The power of two that brings a query row of largest magnitude m into f16's upper range
 // ([2^13, 2^14)); 0 for zeros and non-finite values.
