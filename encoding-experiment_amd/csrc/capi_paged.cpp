@@ -133,6 +133,9 @@ larql::PagedAttnArgs make_attn(const larql_paged_kv* kv, const larql_paged_batch
     const int few = larql::paged_few(a.c, a.kv_type, static_cast<long long>(rows));
     const double groups = bt->q_start ? std::min(n * ((few + most - 1) / most), n + rows / most) : n * ((a.reps + most - 1) / most);
     need(groups * kv->num_kv_heads * (a.c.cap / 32 + 1) < 2147483647.0, "too many positions in one call");
+    // a launch counts its threads in 32 bits: 256 for each segment to join, and for each tile of rows
+    const double segments = n * ((std::max(bt->q_start ? std::min<double>(larql::kPagedFewAll, rows) : a.reps, 1.0) + most - 1) / most);
+    need(std::max(segments, bt->q_start ? n + rows / 128 : 0.0) * kv->num_kv_heads < 16777216.0, "too many rows in one call");
     return a;
 }
 
@@ -150,6 +153,7 @@ extern "C" int larql_hip_paged_append_dev(larql_hip_ctx* c, const larql_paged_kv
         need(num_q_heads <= 65535 && (T == 0 || (num_q_heads == 0) == (q == nullptr)), "q and num_q_heads must come together");
         need(rotary_dim <= hd && rotary_dim % 2 == 0, "rotary_dim must be even and at most head_dim");
         need(std::isfinite(rope_base) && rope_base >= 0.0, "rope_base must be positive, or 0 for no rotation");
+        need(T < (size_t{1} << 26), "too many tokens in one call");  // (a launch counts its threads in 32 bits: 64 a token)
         if (T == 0) return;
         check_rows(k, k_stride, kvd, type, "k");
         check_rows(v, v_stride, kvd, type, "v");

@@ -527,7 +527,7 @@ typedef struct {
  * E4M3 ones are x * (1 / scale), saturated at +-448 (NaN stays NaN).  q NULL (num_q_heads 0): keys
  * and values only.  q_out may be q itself (same stride); otherwise it overlaps none of the others, and nothing
  * overlaps the pages.  A position below 0 or without a page
- * stores nothing, its q row is still rotated.  Two tokens of one call must not share a slot. */
+ * stores nothing, its q row is still rotated.  Two tokens of one call must not share a slot.  Up to 2^26 tokens. */
 int larql_hip_paged_append_dev(larql_hip_ctx* ctx, const larql_paged_kv* cache, const larql_paged_batch* batch,
                                int type, const void* q, size_t q_stride, size_t num_q_heads, const void* k,
                                size_t k_stride, const void* v, size_t v_stride, void* q_out, size_t q_out_stride,
