@@ -383,7 +383,7 @@ struct PagedDecode {
             }
         }
         float x[NC][8], least[NC];
-        bool bands = false;
+        bool small = false, bands = false;  // weights that are too small for the parts; taken apart
 #pragma unroll
         for (int j = 0; j < NC; j++) {
 #pragma unroll
@@ -405,42 +405,46 @@ struct PagedDecode {
                     x[j][e] = (!MULTI || (at >= lo && at < hi)) && (u.ok >> e & 1) ? x[j][e] : -INFINITY;
                 }
             }
-            float mx = x[j][0], mn = x[j][0];
+            float mx = x[j][0];
 #pragma unroll
             for (int e = 1; e < 8; e++) mx = fmaxf(mx, x[j][e]);
-            if constexpr (!BF) {
-#pragma unroll
-                for (int e = 1; e < 8; e++) mn = fminf(mn, x[j][e]);
-                if (edge) {  // of the attended ones
-                    mn = INFINITY;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) mn = fminf(mn, x[j][e] == -INFINITY ? INFINITY : x[j][e]);
-                }
-            }
             mx = max_x32(max_x16(mx)) * f;
-            const bool under = Weights::under(mx, st.m[j]);
-            if (__any(under || Weights::above(mx, st.m[j]))) {
-                const float was = st.m[j];
-                st.m[j] = Weights::reference(mx, was);
-                if (__any(under)) {
-                    const float d = room(st, j, under ? was - ceilf(mx) : 0.f);
-                    if (under) st.m[j] = was - d;
-                }
-                scale(st, j, exp2_hw(was - (st.m[j] == -INFINITY ? 0.f : st.m[j])));
-            }
-            least[j] = INFINITY;
-            if constexpr (!BF) {
-                const float up = Weights::offset(st.m[j]), z = __builtin_fmaf(mn, f, up);
-                if (!Weights::far(st.m[j])) least[j] = z;
-                if (__any(least[j] < Weights::LEAST)) {
-                    float larger = 0.f, seen = 0.f;
+            // (of a whole unit eight positions of the column, more than there may be larger weights: one of them tells)
+            static_assert(Weights::FEW < 8, "");
+            float mn = fminf(x[j][0], x[j][1]);
+            if (!BF && edge) {
+                mn = INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        larger += __builtin_fmaf(x[j][e], f, up) < Weights::LEAST ? 0.f : 1.f;
-                        seen += x[j][e] == -INFINITY ? 0.f : 1.f;
+                for (int e = 0; e < 8; e++) mn = fminf(mn, x[j][e] == -INFINITY ? INFINITY : x[j][e]);
+            }
+            const bool under = Weights::under(mx, st.m[j]), moves = under || Weights::above(mx, st.m[j]);
+            if (__any(moves || Weights::tiny(mn, f, st.m[j]))) {
+                if (__any(moves)) {
+                    const float was = st.m[j];
+                    st.m[j] = Weights::reference(mx, was);
+                    if (__any(under)) {
+                        const float d = room(st, j, under ? was - ceilf(mx) : 0.f);
+                        if (under) st.m[j] = was - d;
                     }
-                    bands |= __any(least[j] < Weights::LEAST && Weights::few(sum_x32(sum_x16(larger)), sum_x32(sum_x16(seen))));
+                    scale(st, j, exp2_hw(was - (st.m[j] == -INFINITY ? 0.f : st.m[j])));
                 }
+                small |= __any(Weights::tiny(mn, f, st.m[j]));
+            }
+        }
+        if (!BF && small) {
+#pragma unroll
+            for (int j = 0; j < NC; j++) {
+                const float f = a.softcap > 0.f ? 1.f : st.qf[j], up = Weights::offset(st.m[j]);
+                float mn = INFINITY, larger = 0.f, seen = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const bool in = x[j][e] != -INFINITY;
+                    mn = fminf(mn, in ? x[j][e] : INFINITY);
+                    seen += in ? 1.f : 0.f;
+                    larger += __builtin_fmaf(x[j][e], f, up) < Weights::LEAST ? 0.f : 1.f;
+                }
+                least[j] = Weights::far(st.m[j]) ? INFINITY : __builtin_fmaf(mn, f, up);
+                bands |= __any(least[j] < Weights::LEAST && Weights::few(sum_x32(sum_x16(larger)), sum_x32(sum_x16(seen))));
             }
         }
         // The weights from 2^LEAST on; then, with the sums raised, those below, a band at a time (rare: PagedWeights).

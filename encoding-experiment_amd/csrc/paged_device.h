@@ -302,8 +302,14 @@ struct PagedWeights {
     static __device__ __forceinline__ float before(float up, float raise, float most) {
         return raise == 0.f ? -INFINITY : raise <= most ? up - BAND : INFINITY;
     }
-    // Whether `larger` of a tile's `seen` weights, those that are not too small, are few.
-    static __device__ __forceinline__ bool few(float larger, float seen) { return larger <= fmaxf(1.f, fminf(FEW, 0.25f * seen)); }
+    // Whether a product x (score = x f) has a weight that is too small for the parts.
+    static __device__ __forceinline__ bool tiny(float x, float f, float m) {
+        return !BF && __builtin_fmaf(x, f, offset(m)) < LEAST;
+    }
+    // Whether `larger` of a tile's `seen` weights, those that are not too small, are few (and not all).
+    static __device__ __forceinline__ bool few(float larger, float seen) {
+        return larger < seen && larger <= fmaxf(1.f, fminf(FEW, 0.25f * seen));
+    }
     // Whether a product x (score = x f) is none of the pass at offset up: too small for it, or done at the one before.
     static __device__ __forceinline__ bool other(float x, float f, float up, float before) {
         return __builtin_fmaf(x, f, up) < LEAST || __builtin_fmaf(x, f, before) >= LEAST;

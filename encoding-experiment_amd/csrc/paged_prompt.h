@@ -436,10 +436,10 @@ __global__ __launch_bounds__(256, HD <= 128 && NS <= 2 ? 2 : 1) void paged_promp
                         }
                     }
                 } else if constexpr (!BF) {
+                    // (eight positions of the row, more than there may be larger weights: one of them tells)
+                    static_assert(P::Weights::FEW < 8, "");
 #pragma unroll
-                    for (int j = 0; j < JN; j++)
-#pragma unroll
-                        for (int e = 0; e < 16; e++) mn = fminf(mn, s[j][e]);
+                    for (int e = 1; e < 4; e++) mn = fminf(mn, s[0][e]);
                 }
                 f = a.softcap > 0.f ? 1.f : qf;
                 float mx = s[0][0];
@@ -458,7 +458,7 @@ __global__ __launch_bounds__(256, HD <= 128 && NS <= 2 ? 2 : 1) void paged_promp
                     for (int d = 0; d < DT; d++) o[d] *= al;
                 }
                 up = P::Weights::offset(m);
-                if constexpr (!BF) small = __any(__builtin_fmaf(mn, f, up) < P::Weights::LEAST && !P::Weights::far(m));
+                small = !BF && __any(P::Weights::tiny(mn, f, m));
             }
             if (__builtin_amdgcn_readfirstlane(bad) == it) {  // (the same for the workgroup)
                 if (go)
