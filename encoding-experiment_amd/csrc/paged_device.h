@@ -268,8 +268,8 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 //   every tile 10-40%, in f32 without the matrix cores.
 // With more of them the others stay as they are: taking those apart too cost rows whose scores are spread widely (3 nats
 // deviation) 2 to 5 times the time, for a case in which all of the larger values would have to be near zero.
-// 512 tokens f32 over f16 33.3 us, 41 with a sink 18 nats above the rest, 41 with scores of 3 nats deviation; 32 sequences'
-// decode 53 us in all three.  Without any of it 30 us and 52, and errors of 1e-3 behind a sink of 12 nats, 0.4 at 18.
+// 512 tokens f32 over f16 32 us, 41 with a sink 18 nats above the rest, 40 with scores of 3 nats deviation; 32 sequences'
+// decode 63 us, 1 more with a sink.  Without any of it 30 us and 62, and errors of 1e-3 behind a sink of 12 nats, 0.4 at 18.
 template <bool BF, int NS>
 struct PagedWeights {
     static constexpr float UP = BF ? 0.f : 14.f, LAZY = BF ? 8.f : 1.98f;  // (2^15.98 is f16's largest)

@@ -21,8 +21,8 @@
 //
 // With few tiles the positions of a tile are split over several workgroups and joined in order.
 //
-// Measured, 32 query and 8 kv heads of 128: 8191 tokens bf16 620 us (887 TFLOP/s; its products alone 558,
-// all but them 495), five chunks of up to 1200 tokens behind up to 2500 206 us, 512 tokens f32 over f16 30 us.  Two waves
+// Measured, 32 query and 8 kv heads of 128: 8191 tokens bf16 630 us (870 TFLOP/s; its products alone 558,
+// all but them 495), five chunks of up to 1200 tokens behind up to 2500 209 us, 512 tokens f32 over f16 32 us.  Two waves
 // per SIMD of 32 rows each beat one of 64 rows (half the LDS reads, 732 us): one wave's softmax
 // passes beside the other's products.
 #pragma once
@@ -667,6 +667,8 @@ static void launch_paged_prompt(const PagedAttnArgs& a, hipStream_t s) {
     } else {
         if (act == LARQL_ELEM_F32) paged_prompt_kernel<HD, LARQL_ELEM_BF16, 3><<<grid, block, 0, s>>>(a);
         else if (act == LARQL_ELEM_F16) paged_prompt_kernel<HD, LARQL_ELEM_BF16, 2><<<grid, block, 0, s>>>(a);
+        // (one part of the weights: rounded to 2^-8, results are off by 2.3e-3 where f32 weights give 1.6e-3, most of it
+        // the output's own rounding; with two 8191 tokens take 980 us instead of 638.  Decode, bound by memory, has two.)
         else paged_prompt_kernel<HD, LARQL_ELEM_BF16, 1><<<grid, block, 0, s>>>(a);
     }
     LARQL_HIP_CHECK(hipGetLastError());

@@ -541,8 +541,9 @@ int larql_hip_paged_append_dev(larql_hip_ctx* ctx, const larql_paged_kv* cache, 
  * value that is not finite in one it does attend makes that dim of the row not finite.
  * q, out as for the append; q, out, work and the pages do not overlap.  Results do not depend on the run: no atomics.
  * Softmax statistics and sums are f32.  f32 activations are taken to f32 accuracy over every cache
- * type (f16 and E4M3 pages: each weight to 2^-19 down to 2^-20 of the largest one, and below that
- * where at most four positions of 32 are larger; else to 2^-39 of the row's largest); with 16-bit ones
+ * type (f16 and E4M3 pages: each weight to 2^-19 down to 2^-20 of the largest of its 32 or 64 positions, and
+ * below that where at most four of those, and a quarter, are larger, as beside an attention sink; else to
+ * 2^-39 of the row's largest); with 16-bit ones
  * the weights are rounded to 16 bits (f16, the same with 2^-11 and 2^-28; bf16 over a bf16 cache, two
  * parts of it for one token per sequence).  Weights below 2^-118 of the largest count as 0.
  * work: 16-byte aligned, larql_hip_paged_attention_work_bytes of it, used by this call until it has
