@@ -309,10 +309,10 @@ struct PagedDecode {
             pv_odd<EE + 1>(st, u, sees, at, g);
         }
     }
-    static __device__ __forceinline__ void scale(State& st, int j, float by) {
-        st.l[j] *= by;
+    static __device__ __forceinline__ void scale(State& st, int j, int by) {  // by 2^by
+        st.l[j] = ldexpf(st.l[j], by);
 #pragma unroll
-        for (int e = 0; e < E; e++) st.o[j][e] *= by;
+        for (int e = 0; e < E; e++) st.o[j][e] = ldexp4(st.o[j][e], by);
     }
     // By how much group j's sums may rise, `want` at most.
     static __device__ __forceinline__ float room(const State& st, int j, float want) {
@@ -326,6 +326,7 @@ struct PagedDecode {
         }
         return fmaxf(0.f, fminf(r, want));
     }
+
     static __device__ __forceinline__ void step(State& st, const pg_u4* q_s, Unit& u, const PagedAttnArgs& a,
                                                 const PagedRange& r, int cg, int t, int g, int c) {
         pg_f4 s[NC][2];
@@ -426,7 +427,7 @@ struct PagedDecode {
                         const float d = room(st, j, under ? was - ceilf(mx) : 0.f);
                         if (under) st.m[j] = was - d;
                     }
-                    scale(st, j, exp2_hw(was - (st.m[j] == -INFINITY ? 0.f : st.m[j])));
+                    scale(st, j, sums_move(was, st.m[j]));
                 }
                 small |= __any(Weights::tiny(mn, f, st.m[j]));
             }
@@ -485,12 +486,12 @@ struct PagedDecode {
             if (!__any(more)) break;
             again(u);
 #pragma unroll
-            for (int j = 0; j < NC; j++) scale(st, j, raise < most[j] ? exp2_hw(Weights::BAND) : 1.f);
+            for (int j = 0; j < NC; j++) scale(st, j, raise < most[j] ? static_cast<int>(Weights::BAND) : 0);
             raise += Weights::BAND;
         }
         if (bands) {
 #pragma unroll
-            for (int j = 0; j < NC; j++) scale(st, j, exp2_hw(-most[j]));
+            for (int j = 0; j < NC; j++) scale(st, j, -static_cast<int>(most[j]));
         }
     }
 };
@@ -665,14 +666,13 @@ __global__ __launch_bounds__(64 * paged_wg(MULTI), (PagedDecode<HD, KT, NS, MULT
                 float m = -INFINITY, l = 0.f;
 #pragma unroll
                 for (int w = 0; w < WG; w++) m = fmaxf(m, ml_s[w][col].x);
-                const float mm = m == -INFINITY ? 0.f : m;
                 pg_f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int w = 0; w < WG; w++) {
                     const float2 ml = ml_s[w][col];
-                    const float f = exp2_hw(ml.x - mm);
-                    l += ml.y * f;
-                    o += *reinterpret_cast<const pg_f4*>(o_s + (w * NC * 16 + col) * OP + d) * f;
+                    const int by = sums_move(ml.x, m);
+                    l += ldexpf(ml.y, by);
+                    o += ldexp4(*reinterpret_cast<const pg_f4*>(o_s + (w * NC * 16 + col) * OP + d), by);
                 }
                 if (done) {
                     const int R = 16 * NC * cg + col, tok = paged_div(R, a.rep_mul, a.rep_shift);
@@ -733,19 +733,18 @@ __global__ __launch_bounds__(TH) void paged_decode_join_kernel(PagedAttnArgs a) 
         float m = -INFINITY, l = 0.f;
         for (int i = lane; i < n; i += 64) m = fmaxf(m, ml(i, c).x);
         m = wave_max(m);
-        const float mm = (m == -INFINITY ? 0.f : m) + kJoinDown;
-        for (int i = lane; i < n; i += 64) l += ml(i, c).y * exp2_hw(ml(i, c).x - mm);
+        for (int i = lane; i < n; i += 64) l += ldexpf(ml(i, c).y, sums_move(ml(i, c).x, m) - kJoinDown);
         l = wave_sum(l);
-        if (lane == 0) ml_s[c] = make_float2(mm, l);
+        if (lane == 0) ml_s[c] = make_float2(m, l);
     }
     __syncthreads();
     pg_f4 o = {0.f, 0.f, 0.f, 0.f};
     if (mine) {
-        const float mm = ml_s[col].x;
+        const float m = ml_s[col].x;
 #pragma unroll 4
         for (int i = pg; i < n; i += PG)
-            o += *reinterpret_cast<const pg_f4*>(a.part + static_cast<long long>(part(i, col)) * HD + 4 * d) *
-                 exp2_hw(ml(i, col).x - mm);
+            o += ldexp4(*reinterpret_cast<const pg_f4*>(a.part + static_cast<long long>(part(i, col)) * HD + 4 * d),
+                        sums_move(ml(i, col).x, m) - kJoinDown);
         o_s[k][d] = o;
     }
     __syncthreads();

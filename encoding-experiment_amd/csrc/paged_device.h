@@ -316,8 +316,17 @@ struct PagedWeights {
     }
 };
 
+// The power of two by which sums that stand at reference `from` move to reference `to` (whole numbers; -inf: no sums).  For
+// ldexp, not as a factor: sums of 2^100 may move by less than 2^-126 and be in range still.
+__device__ __forceinline__ int sums_move(float from, float to) {
+    return static_cast<int>(fminf(fmaxf(from - (to == -INFINITY ? 0.f : to), -1000.f), 1000.f));
+}
+__device__ __forceinline__ pg_f4 ldexp4(pg_f4 x, int by) {
+    return pg_f4{ldexpf(x[0], by), ldexpf(x[1], by), ldexpf(x[2], by), ldexpf(x[3], by)};
+}
+
 // Joined parts are taken down by 2^kJoinDown: as many sums as high as they go stay finite.
-constexpr float kJoinDown = 12.f;
+constexpr int kJoinDown = 12;
 
 // Scores are products times `f` >= 0: the query takes the scale's sign, and f stays above 0, so that a masked product
 // of -inf is a score of -inf (of products up to 10^38, over bf16 pages, the least f makes 0).

@@ -452,10 +452,12 @@ __global__ __launch_bounds__(256, HD <= 128 && NS <= 2 ? 2 : 1) void paged_promp
                 if (__any(under || P::Weights::above(mx, m))) {
                     const float was = m, room = P::Weights::room_weights(max_x32(l));
                     m = under ? was - fmaxf(0.f, fminf(was - ceilf(mx), room)) : P::Weights::reference(mx, was);
-                    const float al = exp2_hw(was - (m == -INFINITY ? 0.f : m));
-                    l *= al;
+                    const int al = sums_move(was, m);
+                    l = ldexpf(l, al);
 #pragma unroll
-                    for (int d = 0; d < DT; d++) o[d] *= al;
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], al);
                 }
                 up = P::Weights::offset(m);
                 small = !BF && __any(P::Weights::tiny(mn, f, m));
@@ -639,14 +641,13 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedAttnArgs a)
     if (row < row0 || row >= row0 + n || n * a.reps <= a.few) return;
     float m = -INFINITY, l = 0.f;
     for (int s = 0; s < a.splits; s++) m = fmaxf(m, a.tile_ml[2 * (i * a.splits + s)]);
-    const float mm = (m == -INFINITY ? 0.f : m) + kJoinDown;
     pg_f4 o = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < a.splits; s++) {
         const float2 p = *reinterpret_cast<const float2*>(a.tile_ml + 2 * (i * a.splits + s));
         if (p.y == 0.f) continue;
-        const float f = exp2_hw(p.x - mm);
-        l += p.y * f;
-        o += *reinterpret_cast<const pg_f4*>(a.tile_part + (i * a.splits + s) * HD + 4 * d) * f;
+        const int by = sums_move(p.x, m) - kJoinDown;
+        l += ldexpf(p.y, by);
+        o += ldexp4(*reinterpret_cast<const pg_f4*>(a.tile_part + (i * a.splits + s) * HD + 4 * d), by);
     }
     const float vs = a.kv_type == LARQL_ELEM_E4M3 && a.c.v_scale ? a.c.v_scale[head / a.reps] : 1.f;
     o *= l == 0.f ? 0.f : 1.f / l;
