@@ -445,7 +445,9 @@ struct PagedDecode {
                     larger += __builtin_fmaf(x[j][e], f, up) < Weights::LEAST ? 0.f : 1.f;
                 }
                 least[j] = Weights::far(st.m[j]) ? INFINITY : __builtin_fmaf(mn, f, up);
-                bands |= __any(least[j] < Weights::LEAST && Weights::few(sum_x32(sum_x16(larger)), sum_x32(sum_x16(seen))));
+                larger = sum_x32(sum_x16(larger));  // (by all lanes: those without a position have no small weight)
+                seen = sum_x32(sum_x16(seen));
+                bands |= __any(least[j] < Weights::LEAST && Weights::few(larger, seen));
             }
         }
         // The weights from 2^LEAST on; then, with the sums raised, those below, a band at a time (rare: PagedWeights).
