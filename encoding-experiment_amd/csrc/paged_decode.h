@@ -28,7 +28,7 @@
 //
 // Measured with the join, 8 kv heads of 128 with 4 query heads each: 1 sequence of 131071 positions bf16 106 us (5.1
 // TB/s), 64 of up to 12000 e4m3 159 us (5.1 TB/s), 32 of up to 4096
-// f16 with f32 activations 63 us, 1 of 517 11 us (two launches of 6.7 and 5.5).  8 sequences of 9 new tokens behind up to
+// f16 with f32 activations 63 us, 1 of 517 12 us (two launches of 7.0 and 5.2).  8 sequences of 9 new tokens behind up to
 // 15000 e4m3 positions 54 us, of which 20 are start, changes of segment and the join.
 #pragma once
 
